@@ -536,6 +536,9 @@ __global__ void __launch_bounds__(512, 1)
     g.s_neg = reinterpret_cast<float*>(smp + L::MAX + h * 128);
     g.s_red = reinterpret_cast<float*>(smp + L::RED + h * 1024);
     g.buf = reinterpret_cast<float*>(smp + L::P + h * 8192);
+    // A wait by parity tells a phase from the next one only.  None here can fall further behind: a stage's next fill waits for its
+    // release by all 16 warps, its next release for that fill; a group's next product for all its warps to be ready again, each of
+    // which has waited for the one before; the ring's next return for the copies of the segment it was returned in.
     if (threadIdx.x == 0) {
         for (int i = 0; i < EF_STAGES; i++) {
             bar_init(b_full + 8 * i, 1);
@@ -562,7 +565,8 @@ __global__ void __launch_bounds__(512, 1)
         for (int d = threadIdx.x; d < 16 * DIM / 8; d += 512)
             reinterpret_cast<uint4*>(a.out + t * 16 * DIM)[d] = make_uint4(0, 0, 0, 0);
     uint32_t kq = 0, issued = 0;   // quantized tiles used; tiles fetched (thread 0)
-    uint32_t exacts = 0, cleared = 0;   // segments with exact tiles; those known to be done with the ring (thread 0)
+    bool lent = false;             // exact tiles have borrowed the ring since this head's last quantized one
+    uint32_t taken = 0;            // times it was taken back (thread 0)
     bool ok = true;                // no wait has been given up
 
     volatile EfSeg& seg = *reinterpret_cast<volatile EfSeg*>(smp + L::SEG + h * 64);
@@ -616,11 +620,17 @@ __global__ void __launch_bounds__(512, 1)
             }
             issued++;
         };
-        // exact tiles borrow the ring: copies wait until all heads are done with theirs
-        if (threadIdx.x == 0 && t0 < qend) {
-            bool clear = true;
-            for (; clear && cleared < exacts; cleared++) clear = bar_wait(b_ring, cleared & 1, g.gave_up);
-            for (int k = 0; clear && k < EF_STAGES - 1 && t0 + k < qend; k++) fetch(t0 + k);
+        // exact tiles borrow the ring.  Each warp gives it back where its next segment with quantized tiles begins (the group's
+        // exact tiles are done then), and copies wait until all 16 have.  No head gets past that segment before the copies, so the
+        // barrier is one phase ahead of this wait at most; a count of the segments with exact tiles would be any number ahead, for
+        // the heads walk such segments apart, and a parity cannot tell two phases from none.
+        if (t0 < qend) {
+            if (lent && g.lane == 0) bar_arrive(b_ring);
+            if (threadIdx.x == 0) {
+                const bool clear = !lent || bar_wait(b_ring, taken++ & 1, g.gave_up);
+                for (int k = 0; clear && k < EF_STAGES - 1 && t0 + k < qend; k++) fetch(t0 + k);
+            }
+            lent = false;
         }
         {   // Q': natural dims of chunk c = 4 plane + pair, stored as chunk 4 pair + plane, groups of four as (0, 2, 1, 3)
             const int r = tid >> 2;
@@ -687,10 +697,7 @@ __global__ void __launch_bounds__(512, 1)
         g.np++;
         if (!ok) break;
         tc_fence_after();
-        if (x0 < t1) {
-            exacts++;
-            if (g.lane == 0) bar_arrive(b_ring);
-        }
+        lent |= x0 < t1;
         if (!g.turned) ef_turn<NC>(g.T_O + g.lanes, g.off, g.s_red, g.buf, tid, g.id);
         // sums over the keys
         {

@@ -371,6 +371,10 @@ __global__ void __launch_bounds__((MT + 3) * 128, 1)
                    b_used = bars + 160, b_ph = bars + 168;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int W_PROD = MT * 4, W_MMA = MT * 4 + 8;
+    // A wait by parity tells a phase from the next one only.  None here can fall further behind, since each phase waits for whoever
+    // waits on the one before: a stage is refilled (kf, vf) once the products have released it (ke, ve), which want all builder and
+    // softmax warps' arrivals; scores (s) follow the P of the tile before (ph, p), a segment's queries (q) its last O (o), O's first
+    // product the last one's read-out (of); a raw tile (raw) its readers' release (used); a table (tab) all builders' arrivals.
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
             bar_init(b_q + 8 * i, 4);
