@@ -20,7 +20,7 @@
 // (one DRAM line each), the scales and the rotation rows of the 128 positions.  (Loading them per thread, rows apart, cost 4
 // times the instruction time in L1 wavefronts: 750 us where this form took 652, at 64 rows x 5 queries of 32K.)
 //
-// Rotating is done in packed bf16, as in extend_tc.
+// A rotated pair is summed in 32 bits and rounded once, as in extend_tc (64 rows x 5 queries of 32K 465 us; in packed bf16 439).
 //
 // Measured at 64 rows x 5 queries of 32K: 438 us as a graph, 452 MB at 1.0 TB/s (the floor is 69 us).  The bound is the
 // instructions, about 990 a warp and tile of 32 keys x 20 columns, two fifths of them for the key: 57 % of the issue slots are

@@ -7,8 +7,9 @@
 //
 // A quantized key is the cache's: bf16 after dequantizing.  A 2-bit code left where it lies in its byte is a bf16 subnormal,
 // code 2^(2 plane - 133), so one packed FMA with (scale 2^(119 - 2 plane), offset 2^-14) gives the key times 2^-14, rounded once;
-// the factor goes into c.  Rotating is done in packed bf16, a product rounded before the sum: a key's rotated half carries three
-// bf16 roundings (1.5e-3 of it) where the decode's carries two (1.2e-3), for a third fewer instructions a key.
+// the factor goes into c.  A rotated pair is summed in 32 bits and rounded to bf16 once, so that keys are the decode's bit for bit.
+// (In packed bf16, a product rounded before the sum, a call takes 4 % less, 370 us for 385 at 2,048 queries over 16K, but single
+// rows are then 1.4e-2 off at scores of deviation 3, 5e-2 at 10.)
 // A quantized value is one of two, offset and offset + scale, rounded to f16 (2^-12): the sign of its bit, shifted to the top of
 // its byte, spreads over 16 bits and picks.  P is f16 there (11 bits against bf16's 8), and O stays in the Hadamard domain until
 // the first exact tile or the end, where the row's thread turns its 128 values in tensor memory (a fast Walsh-Hadamard transform
@@ -330,21 +331,18 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) {
     asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(s));
     return d;
 }
-__device__ __forceinline__ uint32_t bf2_mul(uint32_t a, uint32_t b) {
-    uint32_t d;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
-}
-__device__ __forceinline__ uint32_t bf2_neg(uint32_t a) {
-    uint32_t d;
-    asm("neg.bf16x2 %0, %1;" : "=r"(d) : "r"(a));
-    return d;
-}
-// (a, b) -> (a c - b s, b c + a s), packed
+// (a, b) -> (a c - b s, b c + a s) of two pairs: bf16 products are exact in fp32, the sum is rounded there and once to bf16, as the
+// decode rounds a key
 __device__ __forceinline__ void turn_packed(uint32_t& a, uint32_t& b, uint32_t c, uint32_t s) {
-    const uint32_t x = bf2_fma(b, bf2_neg(s), bf2_mul(a, c)), y = bf2_fma(b, c, bf2_mul(a, s));
-    a = x;
-    b = y;
+    asm("{\n\t.reg .b16 a0, a1, b0, b1, c0, c1, s0, s1;\n\t.reg .f32 t, x0, x1, y0, y1;\n\t"
+        "mov.b32 {a0, a1}, %0;\n\tmov.b32 {b0, b1}, %1;\n\tmov.b32 {c0, c1}, %2;\n\tmov.b32 {s0, s1}, %3;\n\t"
+        "fma.rn.f32.bf16 t, b0, s0, 0f00000000;\n\tneg.f32 t, t;\n\tfma.rn.f32.bf16 x0, a0, c0, t;\n\t"
+        "fma.rn.f32.bf16 t, b1, s1, 0f00000000;\n\tneg.f32 t, t;\n\tfma.rn.f32.bf16 x1, a1, c1, t;\n\t"
+        "fma.rn.f32.bf16 t, a0, s0, 0f00000000;\n\tfma.rn.f32.bf16 y0, b0, c0, t;\n\t"
+        "fma.rn.f32.bf16 t, a1, s1, 0f00000000;\n\tfma.rn.f32.bf16 y1, b1, c1, t;\n\t"
+        "cvt.rn.bf16x2.f32 %0, x1, x0;\n\tcvt.rn.bf16x2.f32 %1, y1, y0;\n\t}"
+        : "+r"(a), "+r"(b)
+        : "r"(c), "r"(s));
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {   // NaN if one of them is
     float d;
