@@ -319,11 +319,21 @@ __device__ __forceinline__ bool ef_tile(const ExtendArgs& a, EfGroup<NC>& g, con
         f8_pair(good ? bs : 0u, good ? bl : 0u, vs, vl);
         release();
     }
-    uint32_t bads = 0;
-    if (!QUANT) bads = ef_gather<true>(vr, stage, g.warp, g.lane);
+    bool bad = false;      // the key's value is not finite: zeros stand for it, which no weight of zero turns into NaN
+    if (QUANT) {
+        if (!(vs + vl < INFINITY)) bad = true, vs = vl = 0.0f;
+    } else {
+        bad = ef_gather<true>(vr, stage, g.warp, g.lane) >> g.lane & 1;
+    }
     uint32_t hide = good ? below(kp - t.p0) : 0xffu;
     if (!QUANT && a.P.win && !(a.P.sk && kp < (int)a.P.nsink)) hide |= ~below(kp + (int)a.P.win - t.p0);
     hide &= 0xffu;
+    if (bad) {             // whoever sees it becomes NaN
+        const float nan = __uint_as_float(0x7fc00000u);
+#pragma unroll
+        for (int i = 0; i < NC / 4; i++)
+            if (!((hide >> i) & 1)) g.l[2 * i] = g.l[2 * i + 1] = f2(nan, nan);
+    }
     // ---- weights
     failed |= !warp_wait(g.b_s, g.ns & 1, g.gave_up);
     g.ns++;
@@ -441,12 +451,6 @@ __device__ __forceinline__ bool ef_tile(const ExtendArgs& a, EfGroup<NC>& g, con
             else mma_ss(g.T_O, smem_desc(stage + k * 2048, 16384, 1024), p, D, !begin || k > 0);
         }
         mma_commit(g.b_p);
-    }
-    if (!QUANT && ((bads >> g.lane) & 1)) {   // whoever sees a value that is not finite becomes NaN
-        const float nan = __uint_as_float(0x7fc00000u);
-#pragma unroll
-        for (int i = 0; i < NC / 4; i++)
-            if (!((hide >> i) & 1)) g.l[2 * i] = g.l[2 * i + 1] = f2(nan, nan);
     }
     return true;
 }

@@ -1,0 +1,41 @@
+"""Inputs at the edges of what kv800.extend takes."""
+import ctypes
+
+import pytest
+import torch
+
+import test_extend_gpu as base
+from test_extend_gpu import DEV, Case, close
+
+from lfm3_kv800 import _lib, kv800
+
+pytestmark = pytest.mark.gpu
+
+
+def filled(c, maxq=None, value=float("nan")):
+    """(output, status word) of a call through the C entry into a buffer that holds `value`."""
+    P = c.paged()
+    s, keep = kv800._paged_struct(P, c.q.device, c.qsl.numel() - 1)
+    out = torch.full_like(c.q, value)
+    R, T, maxq = c.qsl.numel() - 1, c.q.shape[0], maxq or max(1, max(c.ql))
+    n = _lib.lib().kv800_extend_workspace_size(R, T, maxq)
+    ws = torch.full((n,), 255, dtype=torch.uint8, device=DEV)
+    cs, sn = (None, None) if c.layer == "slide" else (c.cos.data_ptr(), c.sin.data_ptr())
+    _lib.call("kv800_extend", ctypes.byref(s), c.q.data_ptr(), c.qsl.data_ptr(), R, T, maxq, cs, sn, c.cos.shape[0], out.data_ptr(),
+              ws.data_ptr(), n, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    return out, int(ws[:4].view(torch.int32))
+
+
+@pytest.mark.parametrize("at", [49152, 49664])      # V offsets, V scales
+@pytest.mark.parametrize("n0,ql", [(252, 5), (250, 8), (230, 30), (200, 90)])
+def test_nan_scale_of_a_hidden_key(n0, ql, at):
+    """A V scale or offset that is NaN makes those queries NaN that see its key, in a sub-block that reaches past others."""
+    c = Case("quant", [n0], [ql], nq=[1], seed=ql)
+    ref = c.ref()
+    first = n0 + ql // 2                            # tokens from here on
+    c.qpool[0, at + 2 * first:at + 512] = 0x7f
+    out, status = filled(c)
+    assert status == 0
+    close(out[:ql // 2], ref[:ql // 2])
+    assert torch.isnan(out[ql // 2:]).all()
