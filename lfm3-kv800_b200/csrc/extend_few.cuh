@@ -462,6 +462,7 @@ __device__ __forceinline__ void ef_plan(const ExtendArgs& a, const ExPlan& pl, v
     const int r = threadIdx.x, lane = r & 31, warp = r >> 5;
     ExItem it{};
     int units = 0;
+    if (blockIdx.x == 0) ex_clear_first(a);
     if (r < a.R) {
         const int64_t q0 = a.qsl[r], q1 = a.qsl[r + 1];
         ExRow row;
@@ -563,7 +564,7 @@ __global__ void __launch_bounds__(512, 1)
     pdl_wait();
     pdl_launch_dependents();
     if (a.own) ef_plan(a, pl, reinterpret_cast<volatile int*>(smp + L::RED));
-    // tokens that no row owns
+    // tokens after the last row's, which no row owns
     const int64_t owned = a.R && a.qsl[a.R] > 0 ? a.qsl[a.R] : 0;
     for (int64_t t = owned + (int64_t)blockIdx.x; t < a.T; t += gridDim.x)
         for (int d = threadIdx.x; d < 16 * DIM / 8; d += 512)

@@ -103,4 +103,10 @@ __device__ __forceinline__ bool ex_exact(const ExtendArgs& a, int b, int ns, int
     return true;
 }
 
+// Zeros for the tokens before the first row's, which no row owns, by one CTA: query_start_loc begins with 0 but for odd callers.
+__device__ __forceinline__ void ex_clear_first(const ExtendArgs& a) {
+    const int64_t n = a.R ? min((int64_t)a.qsl[0], a.T) * (QROWS * DIM / 8) : 0;
+    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) reinterpret_cast<uint4*>(a.out)[i] = make_uint4(0, 0, 0, 0);
+}
+
 }  // namespace kv800

@@ -107,6 +107,7 @@ __global__ void __launch_bounds__(1024) extend_plan(const __grid_constant__ Exte
         return plus(warp ? before : 0, lane ? left : 0);
     };
     if (tid == 0) *a.status = 0;
+    ex_clear_first(a);
     __syncthreads();
     int W = 0;
     for (int pass = 0; pass < 2; pass++) {
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__((MT + 3) * 128, 1)
         const int mt = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t S = tmem + lanes + 128 * mt, O = tmem + lanes + 256 + 128 * mt;
-        // tokens that no row owns
+        // tokens after the last row's, which no row owns
         const int64_t owned = a.R && a.qsl[a.R] > 0 ? a.qsl[a.R] : 0;
         for (int64_t t = owned + (int64_t)blockIdx.x; t < a.T; t += gridDim.x)
             for (int d = tid; d < 16 * DIM / 8; d += W_PROD * 32)

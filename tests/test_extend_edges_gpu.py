@@ -39,3 +39,17 @@ def test_nan_scale_of_a_hidden_key(n0, ql, at):
     assert status == 0
     close(out[:ql // 2], ref[:ql // 2])
     assert torch.isnan(out[ql // 2:]).all()
+
+
+@pytest.mark.parametrize("layer", ["quant", "window", "slide"])
+@pytest.mark.parametrize("ql", [[4, 0, 2], [60, 3, 20]])
+def test_tokens_before_the_first_row(layer, ql):
+    """query_start_loc that begins above 0: no row owns the tokens before it, they get zeros."""
+    c = Case(layer, [500, 30, 9], ql, pad=10, seed=2)
+    ref = c.ref()
+    c.qsl += 7
+    c.q = torch.roll(c.q, 7, 0)
+    out, status = filled(c)
+    n = sum(ql)
+    assert status == 0 and (out[:7] == 0).all() and (out[n + 7:] == 0).all()
+    close(out[7:n + 7], ref[:n])
