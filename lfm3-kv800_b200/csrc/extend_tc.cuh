@@ -744,7 +744,8 @@ __global__ void __launch_bounds__((MT + 3) * 128, 1)
                 // a key past the end is hidden by position; its mark would only cost the fast path
                 const uint32_t gone = __ballot_sync(0xffffffffu, in && !kr) & 0xffffu;
                 uint32_t bads = 0;
-                const bool sunk = nsk > 0 && ti == nquant;      // its first keys are the sinks, whose rotation lies apart
+                // its first keys are sinks, whose rotation lies apart: exact key e < nsk at position e
+                const int e0 = (ti - nquant) * EX_TILE, sunk = nsk - e0;
                 const bool next = ti + 1 < walk.t1;
                 if (next) lookup(ti + 1);
                 if (rotate && !warp_wait(b_raw, nraw & 1, gave_up)) goto done;
@@ -760,9 +761,9 @@ __global__ void __launch_bounds__((MT + 3) * 128, 1)
                     if (rotate) {
                         const uint32_t at = sm + L::RAW + r * 64 + (((j >> 1) ^ ((r >> 1) & 3)) << 4) + (j & 1) * 8;
                         c = ld_shared8(at + ExRaw::COS), sn = ld_shared8(at + ExRaw::SIN);
-                        if (sunk && r < nsk && r < a.npos) {
-                            c = __ldg(reinterpret_cast<const uint2*>(a.cos_t + r * 32) + j);
-                            sn = __ldg(reinterpret_cast<const uint2*>(a.sin_t + r * 32) + j);
+                        if (r < sunk && e0 + r < a.npos) {
+                            c = __ldg(reinterpret_cast<const uint2*>(a.cos_t + (int64_t)(e0 + r) * 32) + j);
+                            sn = __ldg(reinterpret_cast<const uint2*>(a.sin_t + (int64_t)(e0 + r) * 32) + j);
                         }
                     }
 #pragma unroll

@@ -53,3 +53,15 @@ def test_tokens_before_the_first_row(layer, ql):
     n = sum(ql)
     assert status == 0 and (out[:7] == 0).all() and (out[n + 7:] == 0).all()
     close(out[7:n + 7], ref[:n])
+
+
+@pytest.mark.parametrize("n0,ql", [([900], [5]), ([900], [90]), ([520, 40], [40, 200]), ([600, 90], [1, 3])])
+@pytest.mark.parametrize("sinks", [100, 128, 129, 200, 300])
+def test_many_sinks(monkeypatch, n0, ql, sinks):
+    """Any number of sinks, those past a tile among them, each rotated by its own position."""
+    monkeypatch.setattr(base, "NSINK", sinks)
+    monkeypatch.setattr(kv800, "NSINK", sinks)
+    c = Case("window", n0, ql, seed=sinks)
+    out, status = filled(c)
+    assert status == 0
+    close(out, c.ref())
