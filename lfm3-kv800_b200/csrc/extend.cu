@@ -181,6 +181,9 @@ extern "C" int kv800_extend(const kv800_paged* P, const uint16_t* q, const int32
         return workspace && workspace_bytes < need ? KV800_ERR_RANGE : KV800_ERR_ARG;
     }
     ExtendArgs a{*P, q, query_start_loc, (int)R, T, max_qlen, cos_t, sin_t, npos, out, (int*)workspace, 0};
+    // positions are below 2^31 - 1, so that no larger window hides and no larger count of sinks shows a key more
+    if (a.P.win > 0x7fffffffLL) a.P.win = 0x7fffffffLL;
+    if (a.P.nsink > 0x7fffffffLL) a.P.nsink = 0x7fffffffLL;
     const Shape sh = shape_of(max_qlen, sm_count(), P->win ? 0 : P->nqmax < (1 << 20) ? P->nqmax * R : 1 << 20);
     a.own = sh.rows == 32 && R <= sh.threads && sh.parts > 1;     // extend_few plans for itself: a row a thread
     const Layout l = layout(R, T, sh);

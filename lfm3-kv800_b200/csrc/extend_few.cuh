@@ -326,7 +326,7 @@ __device__ __forceinline__ bool ef_tile(const ExtendArgs& a, EfGroup<NC>& g, con
         bad = ef_gather<true>(vr, stage, g.warp, g.lane) >> g.lane & 1;
     }
     uint32_t hide = good ? below(kp - t.p0) : 0xffu;
-    if (!QUANT && a.P.win && !(a.P.sk && kp < (int)a.P.nsink)) hide |= ~below(kp + (int)a.P.win - t.p0);
+    if (!QUANT && a.P.win && !(a.P.sk && kp < (int)a.P.nsink)) hide |= ~below((int)min((int64_t)kp - t.p0 + a.P.win, (int64_t)32));
     hide &= 0xffu;
     if (bad) {             // whoever sees it becomes NaN
         const float nan = __uint_as_float(0x7fc00000u);

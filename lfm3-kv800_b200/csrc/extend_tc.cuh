@@ -452,7 +452,7 @@ __global__ void __launch_bounds__((MT + 3) * 128, 1)
                     const int e0 = (quant ? ti : ti - nquant) * EX_TILE, hi = (quant ? p : px) - e0;
                     int lo = 0, ss = 0;
                     if (!quant && a.P.win) {
-                        lo = hi - (int)a.P.win + 1;
+                        lo = max(hi, (int)a.P.win - 1) - (int)a.P.win + 1;
                         ss = a.P.sk ? (int)a.P.nsink - e0 : 0;
                     }
                     const uint32_t* mask = reinterpret_cast<const uint32_t*>(smp + L::MASK + st * 32);

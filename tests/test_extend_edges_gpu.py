@@ -65,3 +65,15 @@ def test_many_sinks(monkeypatch, n0, ql, sinks):
     out, status = filled(c)
     assert status == 0
     close(out, c.ref())
+
+
+@pytest.mark.parametrize("layer", ["window", "slide"])
+@pytest.mark.parametrize("win", [300, 2 ** 31 - 100, 2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 62])
+@pytest.mark.parametrize("ql", [5, 90])
+def test_wide_windows(monkeypatch, layer, win, ql):
+    """A window beyond the row's length, or beyond 32 bits, hides nothing."""
+    monkeypatch.setattr(base, "WIN", win)
+    c = Case(layer, [700, 3], [ql, 2], seed=ql)
+    out, status = filled(c)
+    assert status == 0
+    close(out, c.ref())
