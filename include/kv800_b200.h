@@ -314,8 +314,9 @@ KV800_API int kv800_step_tables(const int32_t* n0, const int32_t* qlen, int64_t 
  * exponentially distributed for a sample of r), r = max(p - q, 0) at the first rejected draft (p without the draft itself
  * when draft_probs is null; p where that leaves nothing) and p of the last row where all stand.  temperature null = 1;
  * 0 = greedy: a draft stands where it is the argmax, and so is the next token.  Ties go to the lowest index.
- * out (R, K + 1) int32: accepted drafts, the next token, -1; emitted (R): how many.  A target row with no finite logit, or
- * with NaN or +inf, accepts nothing and gives no token (greedy: NaN are skipped).  At most 63 drafts a row; a row with more
+ * out (R, K + 1) int32: accepted drafts, the next token, -1; emitted (R): how many.  A target row without a logit above
+ * -inf, or with NaN or +inf, accepts nothing and gives no token.  A greedy row skips NaN and takes +inf as the largest
+ * value; one of -inf and NaN alone gives no token.  At most 63 drafts a row; a row with more
  * than K, or a draft outside [0, V), is flagged in *status (ST_TABLE) and gives nothing, or is rejected there.
  * workspace: kv800_verify_workspace_size(...) bytes, 16-byte aligned, any contents.
  */

@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const __grid_co
 // argmax_v r(v) / e(v) with r = max(p_m - q_m, 0) where draft m was rejected (p_m without d itself, lacking q), r = p_k
 // where all stand, and e = noise[b]: for exponential e that is a sample of r / sum r, without a running sum over the
 // vocabulary whose rounding would decide the token.  T = 0: argmax on both sides.  Ties go to the lowest index.
-// A target row without a finite maximum (everything masked to -inf) accepts nothing and gives no token.
+// A target row without a finite maximum (everything masked to -inf) accepts nothing and gives no token; greedy, +inf is a maximum.
 // Two launches, the second overlapping the first's end.  With q, verify_stats gives the maximum (with its first index) and the sum
 // of exponentials of every slice of every target row, one CTA a slice with all its loads in flight at once; verify_pick, some CTAs a
 // request, merges them, judges the drafts and takes the argmax over one row, which it has to read again: p - q wants the row's sum
@@ -577,7 +577,8 @@ __global__ void __launch_bounds__(VT, 4) verify_pick(const __grid_constant__ Ver
 }
 
 // A slice of a target row without q: its maximum and sum as in Stat, and the winner of the race: v = max (x - m) c - log2 e over
-// the tokens but the row's draft, at i.  Greedy rows race with c = 1 and e = 1: i is the argmax, drafts included.
+// the tokens but the row's draft, at i.  Greedy rows race with c = 1 and e = 1, and with 0 for m, so that +inf wins like any other
+// maximum (inf - inf would take it out): v is the maximum, i the argmax, drafts included, and s means nothing.
 struct Race {
     float m, s, v;
     int i;
@@ -648,7 +649,7 @@ __global__ void __launch_bounds__(VT, 4) verify_race(const __grid_constant__ Ver
         float m = f[0];
 #pragma unroll
         for (int k = 1; k < RE; k++) m = fmaxf(m, f[k]);
-        m = fmaxf(warp_max(m), NEG);
+        m = greedy ? 0.0f : fmaxf(warp_max(m), NEG);
         const f2 m2(-m, -m);
         f2 s2(0.0f, 0.0f);
 #pragma unroll

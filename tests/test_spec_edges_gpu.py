@@ -1,0 +1,49 @@
+"""Inputs at the edges of what spec.verify and spec.step_tables take."""
+import numpy as np
+import pytest
+import torch
+
+from lfm3_kv800 import spec
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("V", [9, 700, 5001])
+def test_greedy_infinities(dtype, probs, V):
+    """Greedy rows with +inf: the first of them is the argmax, whatever the path; NaN are skipped; -inf alone gives nothing."""
+    rs = np.random.RandomState(V)
+    x = torch.randn(12, V, generator=torch.Generator().manual_seed(V)).to(dtype)
+    at = rs.randint(1, V - 1, 12)
+    for i in (0, 2, 3, 6):
+        x[i, at[i]] = float("inf")
+    x[2, at[2] + 1:] = float("inf")                  # several: the first
+    x[3, 0] = float("nan")
+    x[4] = -float("inf")
+    x[5] = torch.finfo(dtype).min                    # equal and finite: the first
+    x[7] = float("nan")
+    x[8, at[8]] = torch.finfo(dtype).max
+    x[9, at[9]], x[9, at[9] + 1] = torch.finfo(dtype).max, float("inf")
+    key = x.double().nan_to_num(nan=-np.inf, posinf=np.inf, neginf=-np.inf)
+    best = [int(r.argmax()) if r.max() > -np.inf else -1 for r in key]
+    for good in (True, False):                       # one draft a row of two target rows
+        tok = torch.zeros(12, dtype=torch.int32)
+        for b in range(6):
+            tok[2 * b + 1] = best[2 * b] if good else (best[2 * b] + 1) % V
+        want = []
+        for b in range(6):
+            if best[2 * b] < 0:
+                want.append([-1, -1])
+            elif good:
+                want.append([best[2 * b], best[2 * b + 1]])
+            else:
+                want.append([best[2 * b], -1])
+        if good:
+            tok = tok.clamp_min(0)
+        q = torch.full((6, V), 1.0 / V, device=DEV) if probs else None
+        t, e = spec.verify(x.to(DEV), tok.to(DEV), torch.arange(0, 13, 2, device=DEV).int(), torch.rand(12, device=DEV),
+                           torch.ones(6, V, device=DEV), 1, q, torch.zeros(6, device=DEV))
+        assert t.tolist() == want
+        assert e.tolist() == [sum(v >= 0 for v in w) for w in want]
