@@ -66,12 +66,12 @@ class Server:
                 vllm_step.write_slots(ev, k, v, p.slots, self.status)
                 t = vllm_step.decode_tables(self.n0, R, self.exact.table, ev.stride(0), self.quant.table, QPAGE, QTOK, self.nqmax)
                 P = kv800.Paged(qpool=self.qv, boff=t["boff"], eoff=t["eoff"], NQ=p.NQ, nqmax=self.nqmax, win=0, **at)
-                y = kv800.extend(P, q, p.query_start_loc, self.cos, self.sin, mql)
+                y = kv800.extend(P, q, p.query_start_loc, self.cos, self.sin, mql, self.status)
             else:                                             # sliding layer: keys are kept rotated, the last 256 are seen
                 vllm_step.write_slots(ev, rope(k, p.positions, self.cos, self.sin), v, p.slots, self.status)
                 t = vllm_step.decode_tables(self.n0, R, self.slide.table, ev.stride(0))
                 P = kv800.Paged(qpool=None, boff=None, eoff=t["eoff"], NQ=self.none, nqmax=0, win=WIN, **at)
-                y = kv800.extend(P, q, p.query_start_loc, None, None, mql)
+                y = kv800.extend(P, q, p.query_start_loc, None, None, mql, self.status)
             x = x + y.float().view(T, 2048) @ self.o[layer]
             x = x / x.square().mean(1, keepdim=True).sqrt()
         spec.commit(s)

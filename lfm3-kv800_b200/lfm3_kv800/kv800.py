@@ -345,7 +345,7 @@ def _decode(P, q, cos_t, sin_t, spb, target, ms):
     return out
 
 
-def extend(P, q, query_start_loc, cos_t, sin_t, max_query_len):
+def extend(P, q, query_start_loc, cos_t, sin_t, max_query_len, status=None):
     """Attention of a chunk of new tokens over the paged cache (prompt chunks, extends, drafted tokens), for a ragged
     batch of rows in one call: the multi-token form of decode().
 
@@ -353,7 +353,8 @@ def extend(P, q, query_start_loc, cos_t, sin_t, max_query_len):
     tokens of its P.N[b].  Each sees the keys at or before its position: sub-blocks below P.NQ[b], the exact pages after
     them (write the chunk's K / V there first: write_slots / write_exact), for P.win only the window and the sinks.
     P.NQ counts the sub-blocks to read quantized, those flushed before the chunk.  max_query_len: host bound of the rows'
-    query counts.  cos_t / sin_t as in decode().  -> (T, 16, 128) bf16; zeros for tokens that no row owns."""
+    query counts.  cos_t / sin_t as in decode().  status: optional device int32 that collects the bits of range checks and of a
+    wait that ran out (16: rows are unwritten).  -> (T, 16, 128) bf16; zeros for tokens that no row owns."""
     if not q.is_cuda:
         _cuda(q, "extend")
     _LAST[0] = _CHOSEN.get("cuda") or _resolve("cuda")
@@ -392,6 +393,8 @@ def extend(P, q, query_start_loc, cos_t, sin_t, max_query_len):
     ws = qsl.new_empty((ws_bytes + 3) >> 2)      # int32 words
     _lib.call("kv800_extend", s, q.data_ptr(), qsl.data_ptr(), R, T, mql, cs, sn, npos, out.data_ptr(), ws.data_ptr(),
               ws_bytes, _raw_stream(dev.index))
+    if status is not None:
+        status.view(-1)[:1].bitwise_or_(ws[:1])
     if _CHECK:
         _check_status(ws[:1], dev, "extend")
     del keep

@@ -77,3 +77,30 @@ def test_wide_windows(monkeypatch, layer, win, ql):
     out, status = filled(c)
     assert status == 0
     close(out, c.ref())
+
+
+@pytest.mark.parametrize("ql", [5, 90])
+def test_status_reaches_the_caller(ql):
+    """A range check that fires inside the call shows in the caller's status word, beside the bits it held, in a graph too."""
+    c = Case("quant", [1500], [ql], seed=16)
+    st = torch.zeros(1, dtype=torch.int32, device=DEV)
+    call = lambda P, status=st: kv800.extend(P, c.q, c.qsl, c.cos, c.sin, ql, status)  # noqa: E731
+    assert torch.equal(call(c.paged()), c.run()) and int(st) == 0
+    P = c.paged()
+    P.boff = c.boff.clone()
+    P.boff[0, 1] = c.qpool.numel()
+    call(P)
+    assert int(st) == 1
+    P = c.paged()
+    P.eoff = c.eoff.clone()
+    P.eoff[0, -1] = c.epool.numel() - 8
+    call(P)
+    assert int(st) == 3
+    call(c.paged())
+    assert int(st) == 3
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(P)
+    st.zero_()
+    g.replay()
+    assert int(st) == 2
