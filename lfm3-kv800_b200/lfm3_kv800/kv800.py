@@ -75,6 +75,24 @@ def _cuda(t, what):
     return t
 
 
+def _on(t, dev, what):
+    """t, a CUDA tensor that has to lie on dev: another GPU's address would be taken for one of dev's."""
+    if isinstance(t, torch.Tensor) and t.device == dev:
+        return t
+    _cuda(t, what)
+    raise RuntimeError(f"{what}: on {t.device}, the other tensors on {dev}")
+
+
+def _status_ptr(status, dev, who):
+    """Address of a status word (a device int32), or None without one."""
+    if status is None:
+        return None
+    _on(status, dev, f"{who} (status)")
+    if status.dtype != torch.int32 or status.numel() < 1:
+        raise ValueError(f"{who}: status must be an int32 tensor, got {status.dtype} {tuple(status.shape)}")
+    return status.data_ptr()
+
+
 def _stream(dev):
     return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
 
@@ -381,12 +399,23 @@ def extend(P, q, query_start_loc, cos_t, sin_t, max_query_len, status=None):
         cs = sn = None
         npos = 0
     else:
-        cs, sn = _bf16(_cuda(cos_t, "extend (cos_t)")), _bf16(_cuda(sin_t, "extend (sin_t)"))
+        cs, sn = _bf16(_on(cos_t, dev, "extend (cos_t)")), _bf16(_on(sin_t, dev, "extend (sin_t)"))
         if cs.dim() != 2 or cs.shape[1] != 32 or sn.shape != cs.shape:
             raise ValueError(f"extend: cos_t / sin_t must be (P, 32), got {tuple(cs.shape)} / {tuple(sn.shape)}")
         npos = cs.shape[0]
         cs, sn = cs.data_ptr(), sn.data_ptr()
-    _cuda(P.epool, "extend (epool)")
+    _status_ptr(status, dev, "extend")
+    _on(P.epool, dev, "extend (epool)")
+    if P.eoff.dim() == 2 and P.eoff.shape[0] < R:
+        raise ValueError(f"extend: eoff has {P.eoff.shape[0]} rows for {R}")
+    if P.win and P.sk is not None:
+        _on(P.sk, dev, "extend (sk)")
+        _on(P.sv, dev, "extend (sv)")
+        for name, t in (("skoff", P.skoff), ("svoff", P.svoff)):
+            if t is not None and t.numel() < R:
+                raise ValueError(f"extend: {name} has {t.numel()} entries for {R} rows")
+    elif not P.win and P.nqmax:
+        _on(P.qpool, dev, "extend (qpool)")
     s, keep = _paged_struct(P, dev, R)
     L = _lib.lib()
     ws_bytes = L.kv800_extend_workspace_size(R, T, mql)

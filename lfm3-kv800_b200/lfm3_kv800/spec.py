@@ -14,7 +14,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .kv800 import _check_status, _cuda, _raw_stream
+from .kv800 import _check_status, _cuda, _on, _raw_stream, _status_ptr
 
 KINDS = {"all": 0, "tail": 1, "window": 2, "flushed": 3}
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -63,31 +63,28 @@ def page_state(rows, pages, device):
     return s
 
 
-def _need(t, name, who, dtype, shape=None):
-    if not t.is_cuda:
-        _cuda(t, f"{who} ({name})")
+def _need(t, name, who, dev, dtype, shape=None):
+    if t.device != dev:
+        _on(t, dev, f"{who} ({name})")
     if t.dtype != dtype or not t.is_contiguous() or (shape is not None and t.shape != shape):
         raise ValueError(f"{who}: {name} must be contiguous {dtype}{'' if shape is None else ' ' + str(shape)}, got "
                          f"{t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
-def _group(g, R, out, who):
-    table, ring, state, kind = g.table, g.ring, g.state, KINDS.get(g.kind)
+def _group(g, R, dev, out, who):
+    table, kind = g.table, KINDS.get(g.kind)
+    if kind is None:
+        raise ValueError(f"{who}: kind {g.kind!r}: expected one of {', '.join(KINDS)}")
+    if table.device != dev:
+        _on(table, dev, f"{who} (table)")
     shape = table.shape
-    if not (kind is not None and len(shape) == 2 and shape[0] == R and table.is_cuda and table.dtype is torch.int32
-            and (table.stride(1) == 1 and (table.stride(0) >= shape[1] or R == 1) or not R) and ring.is_cuda and ring.dtype is torch.int32 and ring.is_contiguous()
-            and state.is_cuda and state.dtype is torch.int64 and state.dim() == 1 and state.numel() == 2 * R + 2
-            and state.is_contiguous()):
-        if kind is None:
-            raise ValueError(f"{who}: kind {g.kind!r}: expected one of {', '.join(KINDS)}")
-        _need(ring, "ring", who, torch.int32)
-        _need(state, "state", who, torch.int64, (2 * R + 2,))
-        _cuda(table, f"{who} (table)")
+    if len(shape) != 2 or shape[0] != R or table.dtype is not torch.int32 or (
+            R and (table.stride(1) != 1 or (table.stride(0) < shape[1] and R > 1))):
         raise ValueError(f"{who}: table must be ({R}, W) int32 with rows of its own and unit column stride, got {table.dtype} "
                          f"{tuple(shape)} with strides {table.stride()}")
-    return _lib.Pages(table.data_ptr(), max(table.stride(0), shape[1]), shape[1], ring.data_ptr(), ring.numel(),
-                      state.data_ptr(), out, g.page_tokens, kind)
+    return _lib.Pages(table.data_ptr(), max(table.stride(0), shape[1]), shape[1], _need(g.ring, "ring", who, dev, torch.int32),
+                      g.ring.numel(), _need(g.state, "state", who, dev, torch.int64, (2 * R + 2,)), out, g.page_tokens, kind)
 
 
 def step_tables(n0, qlen, max_tokens, exact, quant=None, status=None):
@@ -96,11 +93,12 @@ def step_tables(n0, qlen, max_tokens, exact, quant=None, status=None):
     `quant` (a Pages each) in row order, and their tables are filled in place; pages a row no longer needs go back.  The
     groups' states change only with commit(), so a step may be planned again.  status: optional device int32 that
     collects ST_TABLE (8) where a row found no room or the tokens are more than max_tokens.  -> StepTables."""
-    pn = _need(n0, "n0", "step_tables", torch.int32)
-    pl = _need(qlen, "qlen", "step_tables", torch.int32, n0.shape)
-    dev, R, T = n0.device, n0.numel(), int(max_tokens)
+    dev, R, T = _cuda(n0, "step_tables (n0)").device, n0.numel(), int(max_tokens)
+    pn = _need(n0, "n0", "step_tables", dev, torch.int32)
+    pl = _need(qlen, "qlen", "step_tables", dev, torch.int32, n0.shape)
     if T < 0:
         raise ValueError(f"step_tables: max_tokens must not be negative, got {max_tokens}")
+    pst = _status_ptr(status, dev, "step_tables")
     # the results share two buffers: T positions, T slots, the states | T rows, R + 1 starts, R lengths, R sub-block counts
     n = 2 * R + 2
     m = n if quant is None else 2 * n
@@ -108,10 +106,10 @@ def step_tables(n0, qlen, max_tokens, exact, quant=None, status=None):
     wide = exact.state.new_empty(2 * T + m)      # int64, or _group refuses
     w, i = wide.data_ptr(), narrow.data_ptr()
     es = w + 16 * T
-    ge = _group(exact, R, es, "step_tables: exact")
-    gq = None if quant is None else _group(quant, R, es + 8 * n, "step_tables: quant")
+    ge = _group(exact, R, dev, es, "step_tables: exact")
+    gq = None if quant is None else _group(quant, R, dev, es + 8 * n, "step_tables: quant")
     _lib.call("kv800_step_tables", pn, pl, R, T, ge, gq, i + 4 * T, i, w, w + 8 * T, i + 4 * (T + R + 1),
-              i + 4 * (T + 2 * R + 1), None if status is None else status.data_ptr(), _raw_stream(dev.index))
+              i + 4 * (T + 2 * R + 1), pst, _raw_stream(dev.index))
     _check_status(status, dev, "step_tables")
     rows, qsl, N, NQ = narrow.unsafe_split_with_sizes((T, R + 1, R, R))
     pos, slots, est, qst = wide.unsafe_split_with_sizes((T, T, n, m - n))
@@ -145,15 +143,16 @@ def verify(logits, tokens, query_start_loc, uniform, noise, max_drafts, draft_pr
     K, R = int(max_drafts), query_start_loc.numel() - 1
     if R < 0 or K < 0 or V < 1:
         raise ValueError(f"verify: {R} rows, {K} drafts, {V} tokens")
-    pt = _need(tokens, "tokens", "verify", torch.int32, (T,))
-    ps = _need(query_start_loc, "query_start_loc", "verify", torch.int32, (R + 1,))
-    pu = _need(uniform, "uniform", "verify", torch.float32, (T,))
-    pt0 = None if temperature is None else _need(temperature, "temperature", "verify", torch.float32, (R,))
-    noise, ln = _wide(noise, "noise", R, V)
+    pt = _need(tokens, "tokens", "verify", dev, torch.int32, (T,))
+    ps = _need(query_start_loc, "query_start_loc", "verify", dev, torch.int32, (R + 1,))
+    pu = _need(uniform, "uniform", "verify", dev, torch.float32, (T,))
+    pt0 = None if temperature is None else _need(temperature, "temperature", "verify", dev, torch.float32, (R,))
+    pst = _status_ptr(status, dev, "verify")
+    noise, ln = _wide(noise, "noise", dev, R, V)
     nq = lq = pq = None
     if draft_probs is not None:
         nq = draft_probs.shape[0]
-        draft_probs, lq = _wide(draft_probs, "draft_probs", nq, V)
+        draft_probs, lq = _wide(draft_probs, "draft_probs", dev, nq, V)
         pq = draft_probs.data_ptr() or noise.data_ptr()      # no row at all: any address, none is read
     if T > 1 and logits.stride(0) < V:
         logits = logits.contiguous()                         # rows that overlap (expanded)
@@ -162,17 +161,17 @@ def verify(logits, tokens, query_start_loc, uniform, noise, max_drafts, draft_pr
     p = buf.data_ptr()
     _lib.call("kv800_verify", logits.data_ptr(), dtype, max(logits.stride(0), V), T, V, pt, ps, R, K, pu, noise.data_ptr(), ln,
               pq, nq or 0, lq or 0, pt0, p + 4 * words, p + 4 * (words + R * (K + 1)), p, 4 * words,
-              None if status is None else status.data_ptr(), _raw_stream(dev.index))
+              pst, _raw_stream(dev.index))
     _, out, emitted = buf.unsafe_split_with_sizes((words, R * (K + 1), R))
     out = out.view(R, K + 1)
     _check_status(status, dev, "verify")
     return out, emitted
 
 
-def _wide(t, name, rows, V):
+def _wide(t, name, dev, rows, V):
     """A (rows, V) fp32 tensor whose rows do not overlap, and their stride."""
-    if not t.is_cuda:
-        _cuda(t, f"verify ({name})")
+    if t.device != dev:
+        _on(t, dev, f"verify ({name})")
     if t.dtype != torch.float32 or t.shape != (rows, V) or (rows and t.stride(1) != 1):
         raise ValueError(f"verify: {name} must be ({rows}, {V}) fp32 with unit column stride, got {t.dtype} {tuple(t.shape)}")
     if rows > 1 and t.stride(0) < V:
