@@ -298,7 +298,8 @@ typedef struct kv800_pages {
  * and its slot page * page_tokens + position % page_tokens (-1 where the token has no page); N = n0 + qlen and
  * NQ = nq(n0) per row; new pages of both groups from their rings in row order, dead ones back to them.  Running it again
  * before the state is committed gives the same result.  quant may be null.  A row whose new pages the table or the ring
- * has no room for gets none; that, and more than T tokens, set ST_TABLE in *status (an optional device int).
+ * has no room for gets none; that, and more than T tokens, set ST_TABLE in *status (an optional device int).  R = T = 0
+ * is no work: nothing is written.
  */
 KV800_API int kv800_step_tables(const int32_t* n0, const int32_t* qlen, int64_t R, int64_t T, const kv800_pages* exact,
                  const kv800_pages* quant, int32_t* query_start_loc, int32_t* rows, int64_t* positions, int64_t* slots,

@@ -108,6 +108,11 @@ def step_tables(n0, qlen, max_tokens, exact, quant=None, status=None):
     es = w + 16 * T
     ge = _group(exact, R, dev, es, "step_tables: exact")
     gq = None if quant is None else _group(quant, R, dev, es + 8 * n, "step_tables: quant")
+    if not R and not T:      # no work for the library: an empty plan, the groups as they are
+        narrow.zero_()
+        wide[:n].copy_(exact.state)
+        if quant is not None:
+            wide[n:].copy_(quant.state)
     _lib.call("kv800_step_tables", pn, pl, R, T, ge, gq, i + 4 * T, i, w, w + 8 * T, i + 4 * (T + R + 1),
               i + 4 * (T + 2 * R + 1), pst, _raw_stream(dev.index))
     _check_status(status, dev, "step_tables")

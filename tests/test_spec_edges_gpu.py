@@ -47,3 +47,16 @@ def test_greedy_infinities(dtype, probs, V):
                            torch.ones(6, V, device=DEV), 1, q, torch.zeros(6, device=DEV))
         assert t.tolist() == want
         assert e.tolist() == [sum(v >= 0 for v in w) for w in want]
+
+
+def test_no_rows_and_no_tokens():
+    """A step of nothing leaves the groups as they are."""
+    g = spec.Pages(torch.zeros(0, 4, dtype=torch.int32, device=DEV), torch.arange(8, device=DEV).int(), spec.page_state(0, 8, DEV), 64)
+    none = torch.zeros(0, dtype=torch.int32, device=DEV)
+    for quant in (None, spec.Pages(g.table, g.ring, spec.page_state(0, 5, DEV), 1280, "flushed")):
+        junk = [torch.full((64,), -1, dtype=d, device=DEV) for d in (torch.int32, torch.int64) for _ in range(8)]
+        del junk                                     # what a new buffer is made of
+        s = spec.step_tables(none, none, 0, g, quant)
+        assert s.query_start_loc.tolist() == [0] and s.exact_state.tolist() == [0, 8]
+        spec.commit(s)
+        assert g.state.tolist() == [0, 8] and (quant is None or quant.state.tolist() == [0, 5])
