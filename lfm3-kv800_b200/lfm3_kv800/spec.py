@@ -162,12 +162,11 @@ def verify(logits, tokens, query_start_loc, uniform, noise, max_drafts, draft_pr
     if T > 1 and logits.stride(0) < V:
         logits = logits.contiguous()                         # rows that overlap (expanded)
     words = _lib.lib().kv800_verify_workspace_size(R, min(K, MAX_DRAFTS), V) >> 2
-    buf = tokens.new_empty(words + R * (K + 2))      # scratch, tokens, counts
-    p = buf.data_ptr()
+    scratch, buf = tokens.new_empty(words), tokens.new_empty(R * (K + 2))      # buf: tokens, counts
+    p, n = buf.data_ptr(), R * (K + 1)
     _lib.call("kv800_verify", logits.data_ptr(), dtype, max(logits.stride(0), V), T, V, pt, ps, R, K, pu, noise.data_ptr(), ln,
-              pq, nq or 0, lq or 0, pt0, p + 4 * words, p + 4 * (words + R * (K + 1)), p, 4 * words,
-              pst, _raw_stream(dev.index))
-    _, out, emitted = buf.unsafe_split_with_sizes((words, R * (K + 1), R))
+              pq, nq or 0, lq or 0, pt0, p, p + 4 * n, scratch.data_ptr(), 4 * words, pst, _raw_stream(dev.index))
+    out, emitted = buf.unsafe_split_with_sizes((n, R))
     out = out.view(R, K + 1)
     _check_status(status, dev, "verify")
     return out, emitted

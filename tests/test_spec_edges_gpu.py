@@ -60,3 +60,15 @@ def test_no_rows_and_no_tokens():
         assert s.query_start_loc.tolist() == [0] and s.exact_state.tolist() == [0, 8]
         spec.commit(s)
         assert g.state.tolist() == [0, 8] and (quant is None or quant.state.tolist() == [0, 5])
+
+
+@pytest.mark.parametrize("probs", [False, True])
+def test_verify_results_hold_no_scratch(probs):
+    """A result that is kept does not keep the call's workspace."""
+    R, K, V = 8, 4, 60000
+    x = torch.randn(R * (K + 1), V, device=DEV)
+    q = torch.softmax(torch.randn(R * K, V, device=DEV), -1) if probs else None
+    t, e = spec.verify(x, torch.zeros(R * (K + 1), dtype=torch.int32, device=DEV), torch.arange(0, R * (K + 1) + 1, K + 1, device=DEV).int(),
+                       torch.rand(R * (K + 1), device=DEV), torch.ones(R, V, device=DEV), K, q)
+    for y in (t, e):
+        assert y.untyped_storage().nbytes() <= 4 * R * (K + 2) + 512
