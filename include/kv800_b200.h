@@ -264,7 +264,9 @@ KV800_API int kv800_combine(const float* mo, const float* lo, const float* ao, i
  * and for win > 0 only the last win positions plus, with sinks, the positions < nsink: those before every query's window
  * from sk / sv, the others from the pages.  NQ[b] is the count of sub-blocks flushed before the chunk; a sub-block that
  * reaches past a query's position is masked by position like any other key.  A query without a key, and the tokens that
- * no row owns (i < query_start_loc[0] or i >= query_start_loc[R]), get zeros.  cos_t / sin_t as for kv800_decode.
+ * no row owns (i < query_start_loc[0] or i >= query_start_loc[R]), get zeros.  A V row with a value that is not
+ * finite makes its whole head NaN for every query that sees it; what a query does not see, finite or not, leaves it
+ * alone.  cos_t / sin_t as for kv800_decode.
  * max_qlen: host bound of the rows' query counts (longer rows are cut to it and flagged in the status word).
  * workspace: kv800_extend_workspace_size(...) bytes, 256-byte aligned, any contents; its first int is the status word.
  */

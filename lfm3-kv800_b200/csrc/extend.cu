@@ -25,13 +25,14 @@ int sm_count() {
 }
 
 // The kernel by the longest row.  Up to 6 queries (24 rows a KV head) extend_few, whose cost is the keys': 64 rows x 5 queries of
-// 32K take 438 us there and 1,050 on 128-row tiles, of 2K 65 and 92, on a window layer 29 and 37 (a single row 37 and 35 at 32K, 21
-// and 17 on a window layer, but a launch more).  7 and 8 queries, whose sums no longer fit its registers, only over many sub-blocks:
-// 64 x 8 of 32K 724 and 1,051, 16 x 8 228 and 279, but 4 x 8 92 and 84, 64 x 8 of 2K 103 and 93, of a window layer 43 and 39.  Above
-// that the 128-row tile (32 queries), and two of them above 32 (16 rows of 32K x 16 queries: 281 us in one, 304 in two; x 33: 540
-// and 329).
+// 32K take 467 us there and 1,073 on 128-row tiles, of 2K 67 and 92, on a window layer 31 and 37 (a single row 39 and 36 at 32K, 22
+// and 18 on a window layer, but a launch more).  7 and 8 queries, whose sums no longer fit its registers, only over many sub-blocks:
+// 64 x 8 of 32K 753 and 1,081, 16 x 8 228 and 285, but 4 x 8 96 and 85, 64 x 8 of 2K 101 and 92, of a window layer 42 and 37.  The
+// host knows the sub-blocks by their bound nqmax alone: where that is far above what the rows hold, as in a captured step, 7 and 8
+// queries of short rows take the slower of these.  Above that the 128-row tile (32 queries), and two of them above 32 (16 rows of
+// 32K x 16 queries: 287 us in one, 308 in two; x 33: 551 and 331).
 // Counting what an item's beginning costs evens the parts out: 4,103 queries from 0, whose first query tiles have a key tile or two,
-// took 199 us with 0 units, 169 with 1, 157 with 2, 160 with 3; 64 rows x 5 queries of a window 39 us with 0, 35 with 1, 43 with 2.
+// take 200 us with 0 units, 168 with 1, 154 with 2, 156 with 3; 64 rows x 5 queries of a window 35 us with 0, 31 with 1, 37 with 2.
 constexpr int EX_LEAD = 2, EX_LEAD_FEW = 1;
 struct Shape {
     int qt, rows, parts, threads, lead;   // queries and rows a tile, parts of the work, threads a CTA, ExPlan::lead
@@ -198,7 +199,7 @@ extern "C" int kv800_extend(const kv800_paged* P, const uint16_t* q, const int32
     }
     const int ctas = sh.parts * HEADS;
     if (sh.rows == 32) {
-        // a tile's scores cost by the column: 64 rows x 5 queries of 32K take 458 us in 20, 477 in 24
+        // a tile's scores cost by the column: 64 rows x 5 queries of 32K take 467 us in 20, 483 in 24
         constexpr int smem = EfSmem::BYTES;
         if (max_qlen <= 4) return launch<extend_few<16>, 32>(sh.parts, smem, a, pl, sh.threads, st, maps);
         if (max_qlen == 5) return launch<extend_few<20>, 32>(sh.parts, smem, a, pl, sh.threads, st, maps);

@@ -20,12 +20,13 @@
 // (one DRAM line each), the scales and the rotation rows of the 128 positions.  (Loading them per thread, rows apart, cost 4
 // times the instruction time in L1 wavefronts: 750 us where this form took 652, at 64 rows x 5 queries of 32K.)
 //
-// A rotated pair is summed in 32 bits and rounded once, as in extend_tc (64 rows x 5 queries of 32K 465 us; in packed bf16 439).
+// A rotated pair is summed in 32 bits and rounded once, as in extend_tc (64 rows x 5 queries of 32K 467 us; in packed bf16 438).
 //
-// Measured at 64 rows x 5 queries of 32K: 438 us as a graph, 452 MB at 1.0 TB/s (the floor is 69 us).  The bound is the
-// instructions, about 990 a warp and tile of 32 keys x 20 columns, two fifths of them for the key: 57 % of the issue slots are
+// Measured at 64 rows x 5 queries of 32K: 467 us as a graph, 452 MB at 0.97 TB/s (the floor is 69 us).  The bound is the
+// instructions, about 1,050 a warp and tile of 32 keys x 20 columns, two fifths of them for the key: 58 % of the issue slots are
 // used by the 16 warps that the registers allow, the rest goes in the chain from key to scores to weights to output.
-// On a window layer (64 x 5, 29 us for 35 MB; 1 x 4, 20 us) a CTA has one or two tiles: latency, with instruction fetch.
+// On a window or sliding layer (64 x 5, 31 us for 35 MB; 1 x 4, 21 us) a CTA has one or two tiles: latency, with instruction fetch.
+// Where other forms' times stand below, they were taken side by side while the rotation was still packed (438 us).
 #pragma once
 #include <cuda.h>
 
@@ -456,8 +457,8 @@ __device__ __forceinline__ bool ef_tile(const ExtendArgs& a, EfGroup<NC>& g, con
 }
 
 // The plan of extend_plan, made by each CTA for its own part, a row a thread (at most 512 rows): one load's latency and two barriers
-// instead of a launch and its results' way through memory.  64 rows x 5 queries of a window take 29 us so, 31
-// with extend_plan, a single row of 4 queries 20.6 and 22.6.
+// instead of a launch and its results' way through memory.  64 rows x 5 queries of a window take 31 us so, 33
+// with extend_plan, a single row of 4 queries 22.4 and 23.7.
 __device__ __forceinline__ void ef_plan(const ExtendArgs& a, const ExPlan& pl, volatile int* sums) {
     const int r = threadIdx.x, lane = r & 31, warp = r >> 5;
     ExItem it{};

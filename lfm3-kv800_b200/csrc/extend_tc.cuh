@@ -20,11 +20,12 @@
 // MMAs, one the TMA copies.
 // The two tiles of MT = 2 take turns: one is in the tensor cores while the other is in the softmax.
 // Bound for long chunks: a tile of 256 rows x 128 keys takes the tensor cores, the exponentials (16 a clock) and the
-// shared-memory and tensor-memory traffic about 2,050 clocks each.  Measured: 2,048 queries over 16,384 tokens more take 371 us,
-// 292 GFLOP at 787 TFLOP/s (48 % of what a cuBLAS bf16 product reaches in a burst), about 6,150 clocks a tile: the tensor cores
+// shared-memory and tensor-memory traffic about 2,050 clocks each.  Measured: 2,048 queries over 16,384 tokens more take 385 us,
+// 292 GFLOP at 758 TFLOP/s (46 % of what a cuBLAS bf16 product reaches in a burst), about 6,400 clocks a tile: the tensor cores
 // are busy for 38 % of it, the issue slots for 54 %; a softmax warp's chain of scores, maximum, exponentials and P is the longest.
-// 4,103 queries from 0 (exact tiles alone, about 6,600 clocks each, and 2.7 item beginnings a CTA) take 148 us, 69 GFLOP at 466.
-// Tried and slower: polynomial exponentials on the FMA pipe (639 us where this took 552), two threads a row (488 / 449), separate
+// 4,103 queries from 0 (exact tiles alone, and 2.7 item beginnings a CTA) take 154 us, 69 GFLOP at 448.  2,048 queries over 2,000
+// tokens more on a window or sliding layer take 43 us.
+// Tried and slower, each beside the form of its day: polynomial exponentials on the FMA pipe (639 us where this took 552), two threads a row (488 / 449), separate
 // loops by template for quantized and exact weights (420 / 386), page lookups two tiles ahead (160 / 153 at 4,103 from 0).
 //
 // Work is cut evenly: the (row, query tile) items are flattened into 128-key tiles and cut into equal parts, each done for the

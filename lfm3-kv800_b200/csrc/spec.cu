@@ -91,7 +91,7 @@ __device__ __forceinline__ void row_pages(const Group& g, int R, int r, uint32_t
 // Bound: a launch and two dependent passes over the rows' lengths and page counts (L2 latency); every CTA scans all rows
 // for itself, which costs less than a second launch up to thousands of rows, and then takes its share of the rows'
 // columns (8 lanes a row) and of the tokens.  8 us for one row, 17 us for 2,048 rows of some 3 tokens, 12 us for 64 rows of some 550
-// (as graphs; a call takes 27 us of the host's time).
+// (as graphs; a call takes 25 us of the host's time).
 __global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const __grid_constant__ TablesArgs a) {
     extern __shared__ uint32_t sm[];
     uint32_t* s_qsl = sm;              // [R + 1]
@@ -315,11 +315,6 @@ __device__ __forceinline__ float rcpf(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float ex2f(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 // running maximum (with its first index) and sum of exp2((x - max) c)
 struct Stat {
@@ -328,7 +323,7 @@ struct Stat {
 };
 __device__ __forceinline__ void merge(Stat& a, const Stat& b, float c) {
     const float m = fmaxf(a.m, b.m);
-    a.s = a.s * ex2f((a.m - m) * c) + b.s * ex2f((b.m - m) * c);   // both finite: NEG stands for "nothing yet"
+    a.s = a.s * exp2_approx((a.m - m) * c) + b.s * exp2_approx((b.m - m) * c);   // both finite: NEG stands for "nothing yet"
     if (b.m > a.m || (b.m == a.m && b.i < a.i)) a.i = b.i;
     a.m = m;
 }
@@ -403,7 +398,7 @@ __global__ void __launch_bounds__(VT) verify_stats(const __grid_constant__ Verif
         if (top > st.m || (top == st.m && at < st.i)) st.i = at;
     }
     st.m = fmaxf(st.m, top);
-    if (edge_at < 0x7fffffff) st.s = ex2f((edge - st.m) * c);
+    if (edge_at < 0x7fffffff) st.s = exp2_approx((edge - st.m) * c);
     const f2 c2(c, c), m2(-st.m, -st.m);
     f2 s2(0.0f, 0.0f);
 #pragma unroll
@@ -415,7 +410,7 @@ __global__ void __launch_bounds__(VT) verify_stats(const __grid_constant__ Verif
             for (int i = 0; i < n; i += 2) {
                 float y, z;
                 mul2(add2(f2(f[i], f[i + 1]), m2), c2).get(y, z);
-                s2 = add2(s2, f2(ex2f(y), ex2f(z)));
+                s2 = add2(s2, f2(exp2_approx(y), exp2_approx(z)));
             }
         }
     {
@@ -501,7 +496,7 @@ __global__ void __launch_bounds__(VT, 4) verify_pick(const __grid_constant__ Ver
     __syncthreads();
     if (d >= 0) {
         const Stat st = s_all[tid];
-        if (greedy ? st.i == d : ud * qd < ex2f((xd - st.m) * c) / st.s) atomicOr(&s_ok, 1ull << tid);
+        if (greedy ? st.i == d : ud * qd < exp2_approx((xd - st.m) * c) / st.s) atomicOr(&s_ok, 1ull << tid);
     }
     __syncthreads();
     const int m = n > 0 ? __ffsll((long long)~s_ok) - 1 : 0;   // accepted drafts (bit n - 1 is never set)
@@ -528,7 +523,7 @@ __global__ void __launch_bounds__(VT, 4) verify_pick(const __grid_constant__ Ver
                 }
 #pragma unroll
                 for (int k = 0; k < PE; k++) {
-                    const float v = fmaf(ex2f((tof(xv[k]) - st.m) * c), inv, -qv[k]) * rcpf(ev[k]);
+                    const float v = fmaf(exp2_approx((tof(xv[k]) - st.m) * c), inv, -qv[k]) * rcpf(ev[k]);
                     if (v > w.v) w = Best{v, (int)j0 + VT * k};   // j grows, so a tie keeps the lower token
                 }
             };
@@ -587,7 +582,7 @@ constexpr int RE = 16;               // tokens a lane
 constexpr int RC = 32 * RE;          // tokens a warp: a slice
 __device__ __forceinline__ void merge(Race& a, const Race& b, float c) {
     const float m = fmaxf(a.m, b.m), fa = (a.m - m) * c, fb = (b.m - m) * c;
-    a.s = a.s * ex2f(fa) + b.s * ex2f(fb);
+    a.s = a.s * exp2_approx(fa) + b.s * exp2_approx(fb);
     const float va = fmaxf(a.v + fa, -INFINITY), vb = fmaxf(b.v + fb, -INFINITY);   // inf - inf: not a candidate
     if (vb > va || (vb == va && b.i < a.i)) a.i = b.i;
     a.v = fmaxf(va, vb);
@@ -657,7 +652,7 @@ __global__ void __launch_bounds__(VT, 4) verify_race(const __grid_constant__ Ver
             const f2 d = add2(f2(f[k], f[k + 1]), m2);
             float y, z;
             mul2(d, c2).get(y, z);
-            s2 = add2(s2, f2(ex2f(y), ex2f(z)));
+            s2 = add2(s2, f2(exp2_approx(y), exp2_approx(z)));
             fma2(d, c2, f2(l[k], l[k + 1])).get(f[k], f[k + 1]);
         }
         if (!greedy && row + 1 < n) {      // the row's draft does not race
@@ -738,7 +733,7 @@ __global__ void __launch_bounds__(VT) race_pick(const __grid_constant__ VerifyAr
     float pd = 0.0f;                 // p of the thread's draft
     if (d >= 0) {
         const Race st = s_all[tid];
-        pd = ex2f((xd - st.m) * c) / st.s;
+        pd = exp2_approx((xd - st.m) * c) / st.s;
         if (greedy ? st.i == d : ud < pd) atomicOr(&s_ok, 1ull << tid);
     }
     __syncthreads();
