@@ -450,14 +450,14 @@ __global__ void __launch_bounds__(VT, 4) verify_pick(const __grid_constant__ Ver
     const bool greedy = c == 0.0f;
     int64_t q0;
     int n = target_rows(a, b, q0);   // k + 1
-    int64_t dq = 0;                  // the request's first row of q: drafts of the rows before it
+    int64_t dq = 0;                  // the request's first row of q: drafts of the rows before it (their tokens less one each)
     {
         int empty = 0;
         for (int base = 0; base < b; base += VT) {
             const int r = base + tid;
             empty += __syncthreads_count(r < b && a.qsl[r + 1] <= a.qsl[r]);
         }
-        dq = q0 - (b - empty);
+        dq = q0 - a.qsl[0] - (b - empty);
     }
     if (n < 0 || dq < 0 || (n && dq + n - 1 > a.nq)) {
         if (tid == 0 && part == 0) flag(a.status, ST_TABLE);

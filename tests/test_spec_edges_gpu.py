@@ -3,6 +3,8 @@ import numpy as np
 import pytest
 import torch
 
+from test_spec_gpu import make, run
+
 from lfm3_kv800 import spec
 
 pytestmark = pytest.mark.gpu
@@ -72,3 +74,18 @@ def test_verify_results_hold_no_scratch(probs):
                        torch.rand(R * (K + 1), device=DEV), torch.ones(R, V, device=DEV), K, q)
     for y in (t, e):
         assert y.untyped_storage().nbytes() <= 4 * R * (K + 2) + 512
+
+
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("first", [1, 3, 40])
+def test_tokens_before_the_first_row(probs, first):
+    """query_start_loc that begins above 0: the drafts' probabilities still begin with the first draft's."""
+    R, K, V = 9, 3, 801
+    x, tok, qsl, u, noise, q, temp = make(R, K, V, torch.float32, probs, 0.2, 11, idle=True)
+    want = run(x, tok, qsl, u, noise, K, q, temp)
+    pad = lambda t: torch.cat((t[:1].expand(first, *t.shape[1:]), t))  # noqa: E731
+    st = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = run(pad(x), pad(tok), qsl + first, pad(u), noise, K, q, temp, st)
+    assert int(st) == 0
+    for a, b in zip(got, want):
+        assert np.array_equal(a, b)
