@@ -266,7 +266,8 @@ KV800_API int kv800_combine(const float* mo, const float* lo, const float* ao, i
  * reaches past a query's position is masked by position like any other key.  A query without a key, and the tokens that
  * no row owns (i < query_start_loc[0] or i >= query_start_loc[R]), get zeros.  A V row with a value that is not
  * finite makes its whole head NaN for every query that sees it; what a query does not see, finite or not, leaves it
- * alone.  cos_t / sin_t as for kv800_decode.
+ * alone.  Scores are 32-bit numbers and weights come from their differences: from about 1e7 in magnitude on these are
+ * rounding errors, as in kv800_decode.  cos_t / sin_t as for kv800_decode.
  * max_qlen: host bound of the rows' query counts (longer rows are cut to it and flagged in the status word).
  * workspace: kv800_extend_workspace_size(...) bytes, 256-byte aligned, any contents; its first int is the status word.
  */
